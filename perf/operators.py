@@ -7,7 +7,6 @@ it makes the calls of ``b200attn``. The sizes are the repository's: 16 query hea
 128 (and the 8 / 2 and 4 / 1 shares of a tensor-parallel rank, and 32 over 8), 36 layers, contexts up
 to 64K tokens, ragged batches of 512 to 16K tokens.
 """
-import functools
 import math
 import os
 import random
@@ -23,7 +22,6 @@ LAYERS = 36      # a page holds the tokens of every layer: 2 * LAYERS planes (K 
 MOST = 64 * 16384 * 512   # K elements of the largest padded batch
 
 
-@functools.cache
 def _b200attn():
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llm-inference_b200")
     if path not in sys.path:
