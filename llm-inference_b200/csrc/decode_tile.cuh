@@ -89,6 +89,8 @@ __device__ __forceinline__ float ex2(float x) {
 // (log2 units): P stays <= 2^8 (exact enough in fp16) and most tiles skip
 // rescaling O.
 constexpr float kRescaleThreshold = 8.f;
+// kWide below: the weights lie 2^kWideShift higher, at most 2^15.
+constexpr float kWideShift = 7.f;
 
 // Scores of one 16-token tile, S^T fragment in the log2 domain. ka/kb: K rows
 // g and g+8 (4 x 16 B at 32j + 8t). With kPartial, rows at or past `valid`
@@ -119,17 +121,27 @@ __device__ __forceinline__ void tile_scores(float (&s)[4], const uint4 (&ka)[4],
 
 // Online softmax + O^T += V^T . P^T for one tile. va: V rows 2t, 2t+1, 2t+8,
 // 2t+9 (2 x 16 B at 64b + 8g); masked rows must hold zeros.
+//
+// P is rounded to 16 bits for the tensor cores: half a step of a weight, 2^-11
+// of it, and where it is subnormal (below 2^-14) 2^-25, so that weights below
+// that are lost. With kWide it is the sum of two 16-bit numbers, P's rounding
+// and the rest, each multiplied (off by 2^-22 of a weight, in place of 2^-11),
+// and the reference kept in m lies kWideShift below the running maximum, which
+// puts what is lost below 2^-32 of the largest weight.
+template <bool kWide = false>
 __device__ __forceinline__ void tile_softmax_pv(WarpState& st, const float (&s)[4], const uint4 (&va)[4][2], int g,
                                                 int t) {
+    constexpr float kShift = kWide ? kWideShift : 0.f;
     float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
     }
-    const bool grow = (mx0 > st.m0 + kRescaleThreshold) || (mx1 > st.m1 + kRescaleThreshold);
+    const bool grow =
+        (mx0 > st.m0 + (kRescaleThreshold + kShift)) || (mx1 > st.m1 + (kRescaleThreshold + kShift));
     if (__any_sync(0xffffffffu, grow)) {
-        const float mn0 = fmaxf(st.m0, mx0), mn1 = fmaxf(st.m1, mx1);
+        const float mn0 = fmaxf(st.m0, mx0 - kShift), mn1 = fmaxf(st.m1, mx1 - kShift);
         const float al0 = ex2(st.m0 - mn0), al1 = ex2(st.m1 - mn1);  // 0 on the first tile
         st.l0 *= al0;
         st.l1 *= al1;
@@ -160,14 +172,24 @@ __device__ __forceinline__ void tile_softmax_pv(WarpState& st, const float (&s)[
     const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
     const uint32_t pb0 = __byte_perm(Xa, Xb, sel);
     const uint32_t pb1 = __byte_perm(Ya, Yb, sel);
+    uint32_t rb0 = 0u, rb1 = 0u;  // what the rounding left
+    if constexpr (kWide) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&X));
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&Y));
+        const uint32_t RX = pack_half2(p0 - x.x, p1 - x.y), RY = pack_half2(p2 - y.x, p3 - y.y);
+        rb0 = __byte_perm(__shfl_sync(0xffffffffu, RX, src_a), __shfl_sync(0xffffffffu, RX, src_b), sel);
+        rb1 = __byte_perm(__shfl_sync(0xffffffffu, RY, src_a), __shfl_sync(0xffffffffu, RY, src_b), sel);
+    }
 
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
         const int b = mt >> 2, q = mt & 3;
         const uint32_t w0 = word(va[0][b], q), w1 = word(va[1][b], q);
         const uint32_t w2 = word(va[2][b], q), w3 = word(va[3][b], q);
-        mma16816(st.o[mt], __byte_perm(w0, w1, 0x5410u), __byte_perm(w0, w1, 0x7632u),
-                 __byte_perm(w2, w3, 0x5410u), __byte_perm(w2, w3, 0x7632u), pb0, pb1);
+        const uint32_t a0 = __byte_perm(w0, w1, 0x5410u), a1 = __byte_perm(w0, w1, 0x7632u);
+        const uint32_t a2 = __byte_perm(w2, w3, 0x5410u), a3 = __byte_perm(w2, w3, 0x7632u);
+        mma16816(st.o[mt], a0, a1, a2, a3, pb0, pb1);
+        if constexpr (kWide) mma16816(st.o[mt], a0, a1, a2, a3, rb0, rb1);
     }
 }
 

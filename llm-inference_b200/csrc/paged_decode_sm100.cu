@@ -29,8 +29,13 @@
 // until the first tile, 5 for flush and join); 256 of one KV head 19.5; a step
 // of 48 with 8 KV heads 78.6 (6.07 TB/s); one of 300 tokens 6.8.
 //
-// P is rounded to 16 bits for the tensor cores (2^-11 of a weight at most, as
-// the output's own rounding); scores, sums, maxima and O stay in 32 bits.
+// The weights go to the tensor cores as two 16-bit numbers each (kWide of
+// tile_softmax_pv: off by 2^-22 of a weight, or by 2^-32 of the largest);
+// scores, sums, maxima and O stay in 32 bits. Against one 16-bit number the
+// eight more products a tile cost 0.1 to 0.3 us where latency counts (one of
+// 300 tokens 7.15 us instead of 7.05, one of 64K 27.4 instead of 27.0, 256 of
+// one KV head 19.6 instead of 19.3) and nothing where HBM does (64 ragged 111.5
+// and 111.6).
 #include <math.h>
 
 #include <algorithm>
@@ -517,7 +522,7 @@ __global__ void __maxnreg__(128)
                     tile_scores<true>(sc, ka, kb, qf, tile_token(g), valid, a.scale_log2);
                     load_v_frags_sw<true>(vt, g, tt, valid, va);
                 }
-                tile_softmax_pv(st, sc, va, g, tt);
+                tile_softmax_pv<true>(st, sc, va, g, tt);
                 // (released as soon as the rows were in registers, a stage made 64 ragged sequences
                 // 112.9 us instead of 111.1)
                 __syncwarp();

@@ -158,6 +158,28 @@ def attend64(q, k, v, heads, kv_heads):
     return out, bound
 
 
+def attend64_wide(q, k, v, heads, kv_heads):
+    """attend64 with the bound of kernels that multiply weights of more than 16 bits.
+
+    A weight p is off by 2^-22 of it (two 16-bit numbers: 2^-11 of what the
+    first leaves, itself 2^-11 of p) or, where that is more, by 2^-25, the
+    largest being at least 2^7: n 2^-32 of the largest |v| in all. Sums of
+    products over 16 tokens are added up in 32 bits: 2^-22 of the sum of sizes
+    for each of n / 16, and for 64 joins of partial sums. The scores, the
+    exponentials and the output's one rounding are as in attend64."""
+    d = q.shape[-1]
+    out, _ = attend64(q, k, v, heads, kv_heads)
+    q, k, v = q.astype(np.float64), k.astype(np.float64), np.abs(v.astype(np.float64))
+    size, _ = attend64(q, k, v, heads, kv_heads)
+    n, g = len(k), heads // kv_heads
+    bound = np.full((heads, d), 2.0 ** -25)
+    for h in range(heads) if n else ():
+        score = (d + 4) * 2.0 ** -24 * (np.abs(k[:, h // g]) @ np.abs(q[h])).max() / np.sqrt(d)
+        bound[h] += (2.0 ** -11 * (1 + 2.0 ** -9) * np.abs(out[h]) + n * 2.0 ** -32 * v[:, h // g].max() +
+                     (2 * score + 2.0 ** -20 + (n / 16 + 64 + 1) * 2.0 ** -22) * size[h])
+    return out, bound
+
+
 def assert_within(got, want, bound):
     got = np.asarray(got, np.float64)
     assert np.all(np.isfinite(got))

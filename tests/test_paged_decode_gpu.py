@@ -7,7 +7,7 @@ import pytest
 import b200attn
 import oracle
 from _gpu import Graph, bits, dev, host
-from _paged import assert_within, attend64, rows_of
+from _paged import assert_within, attend64, attend64_wide, rows_of
 from _util import seeded_f16
 
 pytestmark = pytest.mark.gpu
@@ -288,6 +288,38 @@ def test_flat_and_peaked_scores(cuda, scale):
     c = Cache([1000, 3], 4, 128, 16, 24)
     q = (seeded_f16((2, 2048), 25) * np.float16(scale)).astype(np.float16)
     _check(_decode(c, q, 16), c, q, 16)
+
+
+@pytest.mark.parametrize("H,KVH,d", [(16, 4, 128), (4, 1, 128), (16, 2, 128), (32, 8, 128), (7, 1, 128), (12, 1, 128), (6, 3, 64)])
+def test_weights_keep_more_than_16_bits(cuda, H, KVH, d):
+    """Outputs far below the rows they are made of show the weights' rounding."""
+    lens = [2, 3, 5, 16, 33, 1000]
+    c = Cache(lens, KVH, d, 16, 90)
+    q = seeded_f16((len(lens), H * d), 91, 0.1)
+    got = _decode(c, q, H)
+    for b, n in enumerate(lens):
+        assert_within(got[b], *attend64_wide(q[b].reshape(H, d), c.rows_k(b, n), c.rows_v(b, n), H, KVH))
+
+
+@pytest.mark.parametrize("H,KVH", [(16, 4), (4, 1), (32, 8)])
+def test_many_small_weights_beside_a_large_one(cuda, H, KVH):
+    """2,000 tokens that weigh 2^-26 of the first, whose V row is 0: their sum is the output.
+    200 such sequences, so that a warp meets all tokens of one."""
+    import torch
+    n, B, d = 2000, 200, 128
+    c = Cache([n] * B, KVH, d, 16, 92)
+    c.k[:], c.v[:] = 0, 1
+    q = np.zeros((B, H, d), np.float16)
+    q[:, :, 0] = 8
+    for b in range(B):
+        c.k[c.table[b, 0], 0], c.v[c.table[b, 0], 0] = 25.5, 0
+    c.dk.copy_(torch.from_numpy(c.k))
+    c.dv.copy_(torch.from_numpy(c.v))
+    got = _decode(c, q.reshape(B, -1), H)
+    want, bound = attend64_wide(q[0], c.rows_k(0, n), c.rows_v(0, n), H, KVH)
+    assert want.min() > 2.0 ** -16 > 16 * bound.max()
+    for b in range(B):
+        assert_within(got[b], want, bound)
 
 
 def test_repeated_calls_share_a_workspace(cuda):
