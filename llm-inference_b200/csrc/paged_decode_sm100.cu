@@ -59,6 +59,9 @@ constexpr uint32_t kPtMinPage = 4;
 constexpr uint32_t kPtSmemLimit = 226 * 1024;
 constexpr uint32_t kPtMaxStages = 16;
 constexpr uint32_t kNoSeg = 0xffffffffu;
+// The maximum before any score: below every finite one (a product of 16-bit rows stays within 2^40)
+// and finite itself, so that a score of -infinity (an infinity in K) weighs 0 from the first tile on.
+constexpr float kNoMax = -1e30f;
 // flags kept with a sequence's table row
 constexpr uint32_t kRowBits = 0x0fffffffu, kRowRotate = 1u << 28, kRowAppend = 1u << 29, kRowCapped = 1u << 30;
 
@@ -120,8 +123,8 @@ __device__ __forceinline__ void state_dump(const WarpState& st, float* at) {
 
 __device__ __forceinline__ void join_factors(float& ma, float mb, float& fa, float& fb) {
     const float m = fmaxf(ma, mb);
-    fa = ma == -INFINITY ? 0.f : ex2(ma - m);
-    fb = mb == -INFINITY ? 0.f : ex2(mb - m);
+    fa = ex2(ma - m);
+    fb = ex2(mb - m);
     ma = m;
 }
 
@@ -469,6 +472,7 @@ __global__ void __maxnreg__(128)
             if (fresh) {
                 fresh = false;
                 state_init(st);
+                st.m0 = st.m1 = kNoMax;
                 const uint32_t qs = seg & 1;
                 if (!mbar_wait(&qfull[qs], (seg >> 1) & 1)) {
                     ok = false;
@@ -643,7 +647,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) paged_join_kernel(const Tiled
         x[k] = i < n ? __ldcg(reinterpret_cast<const float4*>(po + i * step)) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const float l0 = tid < n ? __ldcg(pl + tid) : 0.f;
-    float m = -INFINITY;
+    float m = kNoMax;
     for (uint32_t i = tid; i < n; i += kThreads) {
         wgt[i] = __ldcg(pm + i);
         m = fmaxf(m, wgt[i]);
@@ -656,7 +660,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) paged_join_kernel(const Tiled
     for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red[0][w]);
     float l = 0.f;
     for (uint32_t i = tid; i < n; i += kThreads) {
-        const float w = wgt[i] == -INFINITY ? 0.f : ex2(wgt[i] - m);
+        const float w = ex2(wgt[i] - m);
         wgt[i] = w;
         l = fmaf(w, i == tid ? l0 : __ldcg(pl + i), l);
     }

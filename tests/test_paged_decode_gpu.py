@@ -322,6 +322,40 @@ def test_many_small_weights_beside_a_large_one(cuda, H, KVH):
         assert_within(got[b], want, bound)
 
 
+def _formula(c, b, n, q, H):
+    """softmax(q k / sqrt(d)) v of sequence b's first n rows in 64 bits, infinities and NaN as they come."""
+    k, v, g = c.rows_k(b, n).astype(np.float64), c.rows_v(b, n).astype(np.float64), H // c.kvh
+    q, out = q.reshape(H, c.d).astype(np.float64), np.zeros((H, c.d))
+    with np.errstate(all="ignore"):
+        for h in range(H):
+            s = k[:, h // g] @ q[h] / np.sqrt(c.d)
+            p = np.exp(s - s.max())
+            out[h] = (p / p.sum()) @ v[:, h // g]
+    return out
+
+
+@pytest.mark.parametrize("H,KVH,d", [(16, 4, 128), (4, 1, 128), (32, 8, 128), (12, 1, 128), (6, 3, 64), (3, 3, 64)])
+@pytest.mark.parametrize("where", [[0], range(16), range(40, 72), [399]])
+def test_infinities_in_k(cuda, H, KVH, d, where):
+    """A score of -infinity weighs nothing, wherever its tokens lie; one of +infinity has no softmax."""
+    n = 400
+    c = Cache([n, 17], KVH, d, 16, 94)
+    for t in where:
+        c.k[c.table[0, t // 16], t % 16].reshape(KVH, d)[:, 3] = np.inf
+    c.dk.copy_(dev(c.k))
+    q = seeded_f16((2, H * d), 95)
+    got, want = _decode(c, q, H), _formula(c, 0, n, q[0], H)
+    gone = np.isnan(want)
+    assert gone.any() and not gone.all()
+    np.testing.assert_array_equal(np.isnan(got[0]), gone)
+    # the heads that keep a softmax keep its values: those of the other tokens
+    keep = np.setdiff1d(np.arange(n), np.array(where))
+    exact, bound = attend64(q[0].reshape(H, d), c.rows_k(0, n)[keep], c.rows_v(0, n)[keep], H, KVH)
+    fine = ~gone.any(1)
+    assert_within(got[0][fine], exact[fine], bound[fine])
+    _check(got[1:], c, q[1:], H, seqs=[1], lens=[17])
+
+
 def test_repeated_calls_share_a_workspace(cuda):
     """Calls of different lengths on one workspace, on a stream of their own, give what each gives alone."""
     import torch
