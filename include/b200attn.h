@@ -457,7 +457,8 @@ int b2_launch_rope_and_store_kv_paged(void* d_q, const void* d_k, const void* d_
  * ([num_heads][head_dim] fp16 at d_out + b * out_seq_stride) = attention of Q
  * row b (d_q + b * q_seq_stride) over tokens [0, len_b), len_b =
  * clamp(d_kv_len[b] + kv_len_bias, 0, capacity), read at launch (graph
- * static); a length of 0 gives a zero output. d_kv_len is per batch entry, so
+ * static); a length of 0 gives a zero output, so does a head whose scores are
+ * all -infinity; NaN and +infinity scores give NaN. d_kv_len is per batch entry, so
  * several entries may attend different lengths of one sequence (drafted
  * tokens). Strides in elements; 0 = packed.
  * head_dim a multiple of 8 up to 256, num_seqs <= 65535, 16-byte aligned

@@ -31,6 +31,9 @@ constexpr uint32_t kPgUnroll = 4;           // tokens of a lane group in flight
 constexpr uint32_t kPgMaxSplits = 512;
 constexpr uint32_t kPgPart = 192;           // tokens of a part at least
 constexpr uint32_t kPgMergeThreads = 256;
+// The maximum before any score: below every finite one and finite itself, so that a score of -infinity
+// weighs 0, and one that is NaN, which no maximum shows, still makes a NaN of the weight and the output.
+constexpr float kPgNoMax = -1e30f;
 
 struct SplitArgs {
     PagedArgs p;
@@ -101,7 +104,7 @@ __global__ void __launch_bounds__(kPgThreads) paged_split_kernel(const SplitArgs
     float q[G][8], o[G][8], m[G], l[G];
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g) {
-        m[g] = -INFINITY;
+        m[g] = kPgNoMax;
         l[g] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) q[g][i] = o[g][i] = 0.f;
@@ -180,15 +183,14 @@ __global__ void __launch_bounds__(kPgThreads) paged_split_kernel(const SplitArgs
 #pragma unroll
             for (uint32_t u = 0; u < kPgUnroll; ++u)
                 if (in[u]) mn = fmaxf(mn, sc[u][g]);
-            const bool none = mn == -INFINITY;
-            const float c = none ? 1.f : exp2f(m[g] - mn);
+            const float c = exp2f(m[g] - mn);
             m[g] = mn;
             l[g] *= c;
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[g][i] *= c;
 #pragma unroll
             for (uint32_t u = 0; u < kPgUnroll; ++u) {
-                sc[u][g] = in[u] && !none ? exp2f(sc[u][g] - mn) : 0.f;
+                sc[u][g] = in[u] ? exp2f(sc[u][g] - mn) : 0.f;
                 l[g] += sc[u][g];
             }
         }
@@ -220,11 +222,10 @@ __global__ void __launch_bounds__(kPgThreads) paged_split_kernel(const SplitArgs
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < nheads * d; i += kPgThreads) {
         const uint32_t g = i / d, e = i - g * d;
-        float M = -INFINITY, L = 0.f, O = 0.f;
+        float M = kPgNoMax, L = 0.f, O = 0.f;
         for (uint32_t w = 0; w < slots; ++w) M = fmaxf(M, s_m[w * G + g]);
         for (uint32_t w = 0; w < slots; ++w) {
-            const float mw = s_m[w * G + g];
-            const float c = mw == -INFINITY ? 0.f : exp2f(mw - M);
+            const float c = exp2f(s_m[w * G + g] - M);
             L = fmaf(c, s_l[w * G + g], L);
             O = fmaf(c, so[(w * G + g) * d + e], O);
         }
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(kPgMergeThreads) paged_merge_kernel(const Spli
     const uint32_t n = parts_of(t, paged_tokens(a, paged_row(a.pv, b), a.kv_len[b]));
     if (n == 1) return;
     const uint64_t p = (static_cast<uint64_t>(b) * a.num_heads + h) * t.splits;
-    float m = -INFINITY;
+    float m = kPgNoMax;
     for (uint32_t i = tid; i < n; i += kPgMergeThreads) m = fmaxf(m, t.pm[p + i]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
@@ -263,13 +264,13 @@ __global__ void __launch_bounds__(kPgMergeThreads) paged_merge_kernel(const Spli
 #pragma unroll
     for (uint32_t w = 0; w < kPgMergeThreads / 32; ++w) m = fmaxf(m, red[0][w]);
     float l = 0.f;
-    for (uint32_t i = tid; i < n; i += kPgMergeThreads) l = fmaf(m == -INFINITY ? 0.f : exp2f(t.pm[p + i] - m), t.pl[p + i], l);
+    for (uint32_t i = tid; i < n; i += kPgMergeThreads) l = fmaf(exp2f(t.pm[p + i] - m), t.pl[p + i], l);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     if ((tid & 31) == 0) red[1][tid >> 5] = l;
     const uint32_t lanes = a.head_dim / 4, rows = kPgMergeThreads / lanes, r = tid / lanes, e = tid - r * lanes;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < rows && m != -INFINITY) {
+    if (r < rows) {
 #pragma unroll 4
         for (uint32_t i = r; i < n; i += rows) {
             const float c = exp2f(t.pm[p + i] - m);

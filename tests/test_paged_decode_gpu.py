@@ -356,6 +356,25 @@ def test_infinities_in_k(cuda, H, KVH, d, where):
     _check(got[1:], c, q[1:], H, seqs=[1], lens=[17])
 
 
+@pytest.mark.parametrize("H,KVH,d", [(16, 4, 128), (4, 1, 128), (32, 8, 128), (12, 1, 128), (6, 3, 64), (3, 3, 64)])
+def test_nan_in_a_query_reaches_its_output(cuda, H, KVH, d):
+    """All scores of a head are then NaN: so is its output, and no other head's."""
+    lens = [40, 700, 1, 0]
+    c = Cache(lens, KVH, d, 16, 96)
+    q = seeded_f16((4, H * d), 97)
+    nan = [(0, 0), (1, H - 1), (2, H // 2), (3, 0)]
+    for b, h in nan:
+        q[b, h * d + 5] = np.nan
+    got = _decode(c, q, H)
+    for b, h in nan[:3]:
+        assert np.all(np.isnan(got[b, h]))
+        rest = np.arange(H) != h
+        clean = np.nan_to_num(q[b].reshape(H, d))
+        want, bound = attend64(clean, c.rows_k(b, lens[b]), c.rows_v(b, lens[b]), H, KVH)
+        assert_within(got[b][rest], want[rest], bound[rest])
+    assert np.all(got[3] == 0)
+
+
 def test_repeated_calls_share_a_workspace(cuda):
     """Calls of different lengths on one workspace, on a stream of their own, give what each gives alone."""
     import torch
