@@ -465,11 +465,10 @@ __device__ uint32_t extend_plan(ExtendShared& sm, const Seqs& q, const int32_t* 
     } else if (i == 0) {
         tell(head, 0);  // nothing for the others to do
     }
-    // an item that takes more than the pool has ends the call here, so that the sum stays within 32 bits
+    // an item takes table_stride <= kMaxPages pages at most (a copied one held one before), so the sum fits 32 bits
     const uint32_t need = bad ? 0u : want - held + (cow ? 1u : 0u);
-    const bool huge = __syncthreads_or(need > q.num_pages) != 0;
     uint32_t total, copies = 0, place = 0;
-    const uint32_t base = block_scan(huge ? 0u : need, sm.s.scan, total);
+    const uint32_t base = block_scan(need, sm.s.scan, total);
     if (any_cow) place = block_scan(cow ? 1u : 0u, sm.s.scan, copies);
     if (i < n) {
         sm.s.base[i] = base;
@@ -481,9 +480,10 @@ __device__ uint32_t extend_plan(ExtendShared& sm, const Seqs& q, const int32_t* 
     __syncthreads();
     // the free pages, by rank; the first kFound are kept, so that few are looked up twice
     uint32_t* found = reinterpret_cast<uint32_t*>(&sm.s.hash);
-    const bool room = !huge && !bad && free_pages(q, mask0, total, sm.s.scan, [&](uint32_t r, uint32_t page) {
-                                           if (r < kFound) found[r] = page;
-                                       }) == total;
+    auto keep = [&](uint32_t r, uint32_t page) {
+        if (r < kFound) found[r] = page;
+    };
+    const bool room = !bad && total <= q.num_pages && free_pages(q, mask0, total, sm.s.scan, keep) == total;
     __syncthreads();
     if (room) {
         auto give = [&](uint32_t r, uint32_t page) {
@@ -513,7 +513,7 @@ __device__ uint32_t extend_plan(ExtendShared& sm, const Seqs& q, const int32_t* 
     if (i < n && first) first[i] = room && s >= 0 ? old : kNone;
     if (i == 0 && status) {
         status[0] = bad ? B2_PAGES_BAD_ITEM : room ? B2_PAGES_OK : B2_PAGES_SHORT;
-        status[1] = static_cast<int32_t>(huge ? 0x7fffffffu : min(total, 0x7fffffffu));
+        status[1] = static_cast<int32_t>(min(total, 0x7fffffffu));
     }
     copies = room ? copies : 0u;
     __syncthreads();

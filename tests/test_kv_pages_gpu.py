@@ -336,6 +336,26 @@ def test_the_pages_taken_do_not_wrap(cuda):
     assert not length.any() and not ref.any()
 
 
+def test_the_pages_taken_are_counted_when_they_are_too_many(cuda):
+    """Whatever one item asks for, up to a table's width: the count is that of the call."""
+    m = _model(1, 16, 1, 8, 5, 1 << 20)
+    d = Device(m)
+    for seqs, take in (([0], [17]), ([0], [16]), ([1], [1]), ([0, 1, 2], [1, 17, 40]), ([3, 1], [1 << 20, 0]),
+                       ([4, 3, 2, 1], [1 << 20, 1 << 20, (1 << 20) - 5, 3])):
+        got, want = d.extend(seqs, take), m.extend(seqs, take)
+        assert got[:2] == want[:2]
+        np.testing.assert_array_equal(got[2], want[2])
+        d.same()
+    # a copied last page counts too
+    m = _model(1, 3, 4, 8, 3, 8)
+    d = Device(m)
+    for s in (m, d):
+        s.extend([0], [6])
+        s.fork([0], [1])
+    assert d.extend([1], [20])[:2] == m.extend([1], [20])[:2] == (m.SHORT, 6)
+    d.same()
+
+
 def test_on_another_stream_and_captured(cuda):
     """A scheduler's step (drop, fork, extend) captured once, replayed with other items in the same buffers."""
     import torch
