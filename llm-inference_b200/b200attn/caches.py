@@ -66,8 +66,8 @@ class PagedKVCache:
     The state lies on the device (page_table, seq_len, ref_count), and so do the
     operations' arguments: contiguous int32 tensors of table rows, lengths and
     counts on the same device (pos and the arrays after the first may be longer). The
-    operations are launches (no synchronisation, capturable); ``check`` reads the
-    status of the last one. Calls are ordered on one stream, or by the caller.
+    operations are launches (no synchronisation, capturable); ``check`` waits for the
+    last one and reads its status. Calls are ordered on one stream, or by the caller.
     """
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
@@ -92,6 +92,7 @@ class PagedKVCache:
         if self._ws_bytes == 0:
             raise ValueError(f"{num_pages} pages: 1 to 2**21 are possible")
         self._ws = torch.zeros(self._ws_bytes, dtype=torch.uint8, device=device)
+        self._stream = None   # the last operation's
 
     def get_k_pages(self, layer: int):
         """[num_pages, page_size, kv_dim] K pages of a layer."""
@@ -134,12 +135,18 @@ class PagedKVCache:
     def _work(self, stream):
         return self.status, self._ws, self._ws_bytes, stream
 
+    def _launched(self, n, stream):
+        """An operation of n items went to this stream (one without items goes nowhere)."""
+        if n:
+            self._stream = stream
+
     def extend(self, seqs, new_tokens, pos=None, stream=None):
         """Room for new_tokens[i] more tokens of sequence seqs[i]; pos[i] = its first new position."""
         from .kernels import launch_kv_pages_extend
         n = self._items(seqs, new_tokens, pos)
         launch_kv_pages_extend(*self._pool(), *self._table(), self.seq_len, self.ref_count, seqs, new_tokens,
                                n, pos, *self._work(stream))
+        self._launched(n, stream)
 
     def truncate(self, seqs, new_len=None, stream=None):
         """Sequence seqs[i] keeps its first new_len[i] tokens (None: it is freed)."""
@@ -147,6 +154,7 @@ class PagedKVCache:
         n = self._items(seqs, new_len)
         launch_kv_pages_truncate(*self._table(), self.num_pages, self.seq_len, self.ref_count, seqs, new_len,
                                  n, *self._work(stream))
+        self._launched(n, stream)
 
     def fork(self, parents, children, fork_len=None, stream=None):
         """Empty sequence children[i] shares the first fork_len[i] tokens (None: all) of parents[i]."""
@@ -154,6 +162,7 @@ class PagedKVCache:
         n = self._items(parents, children, fork_len)
         launch_kv_pages_fork(*self._table(), self.num_pages, self.seq_len, self.ref_count, parents, children,
                              fork_len, n, *self._work(stream))
+        self._launched(n, stream)
 
     def compact(self, stream=None):
         """Brings the live pages together at the low numbers; status[1] = how many they are."""
@@ -161,20 +170,30 @@ class PagedKVCache:
         self._current()
         launch_kv_pages_compact(*self._pool(), self.page_table, *self._table(), self.seq_len, self.ref_count,
                                 self.ref_count, *self._work(stream))
+        self._launched(1, stream)
 
     def copy_pages(self, src, dst, stream=None):
         """Contents of page dst[i] = those of page src[i], every layer."""
         from .kernels import launch_kv_pages_copy
         launch_kv_pages_copy(*self._pool(), src, dst, self._items(src, dst), stream)
 
-    def check(self):
-        """Raises if the last truncate, fork or extend was refused (synchronises); returns status[1]."""
+    def check(self, stream=None):
+        """Raises if the last truncate, fork or extend was refused; returns status[1]. Waits for the stream that the
+        last operation was launched on, or for ``stream``: the one that a graph of captured operations runs on."""
+        import torch
+        device = self.page_table.device
+        stream = self._stream if stream is None else stream
+        if device.type == "cuda":
+            handle = stream if stream is None or isinstance(stream, int) else stream.cuda_stream
+            (torch.cuda.ExternalStream(handle, device=device) if handle
+             else torch.cuda.default_stream(device)).synchronize()
         code, count = self.status.tolist()
         if code == 1:
             raise MemoryError(f"too few free pages: the call takes {count}")
         if code != 0:
-            raise ValueError("bad item: a row outside the table, a sequence named twice, a length out of range or a "
-                             "child that is not empty")
+            raise ValueError("bad item: a row outside the table, a sequence named twice, a length out of range, a "
+                             "child that is not empty, or a partly filled last page that is outside the pool or "
+                             "without a reference")
         return count
 
 

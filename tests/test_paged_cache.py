@@ -158,6 +158,64 @@ def test_cpp_class_on_a_non_blocking_stream(cuda, tmp_path):
     assert res.returncode == 0, res.stdout + res.stderr
 
 
+def _slow(stream):
+    """Ordinary work of some 30 ms on a stream."""
+    import torch
+    with torch.cuda.stream(stream):
+        a = torch.randn(8192, 8192, device="cuda", dtype=torch.bfloat16)
+        for _ in range(40):
+            a = (a @ a).clamp(-1, 1)
+    return a
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["stream", "handle", "default", "graph"])
+def test_check_waits_for_the_last_operation(cuda, how):
+    """Queued behind slow work on a stream that torch's own does not wait for: its refusal is seen."""
+    import torch
+    from _gpu import Graph
+
+    def ints(x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+    c = b200attn.PagedKVCache(1, 4, 16, 1, 8, 2, 8)
+    one, other, few, many, far = ints([0]), ints([1]), ints([3]), ints([100]), ints([1000])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        if how == "graph":
+            g = Graph()
+            with g:
+                c.extend(one, many, stream=g.stream)
+            keep = _slow(g.stream)
+            assert int(g.rt.cudaGraphLaunch(g.exec, g.stream.cuda_stream)[0]) == 0
+            with pytest.raises(MemoryError, match="takes 7"):
+                c.check(g.stream)
+            g.close()
+            return
+        side = torch.cuda.default_stream() if how == "default" else torch.cuda.Stream()
+        stream = {"stream": side, "handle": side.cuda_stream, "default": None}[how]
+        keep = _slow(side)
+        c.extend(one, many, stream=stream)
+        c.truncate(one[:0], stream=torch.cuda.Stream())      # no items: not an operation
+        with pytest.raises(MemoryError, match="takes 7"):
+            c.check()
+        keep = _slow(side)
+        c.extend(other, few, stream=stream)
+        assert c.check() == 1
+        keep = _slow(side)
+        c.truncate(one, many, stream=stream)
+        with pytest.raises(ValueError, match="length out of range"):
+            c.check()
+        keep = _slow(side)
+        c.extend(other, far, stream=stream)
+        with pytest.raises(ValueError, match="without a reference"):
+            c.check()
+        keep = _slow(side)
+        c.compact(stream=stream)
+        assert c.check() == 1
+    del keep
+
+
 @pytest.mark.gpu
 def test_operations(cuda):
     import torch
