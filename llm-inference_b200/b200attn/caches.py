@@ -93,6 +93,8 @@ class PagedKVCache:
             raise ValueError(f"{num_pages} pages: 1 to 2**21 are possible")
         self._ws = torch.zeros(self._ws_bytes, dtype=torch.uint8, device=device)
         self._stream = None   # the last operation's
+        if self._ws.is_cuda:   # written before a stream that does not wait for torch's uses them
+            torch.cuda.current_stream(self._ws.device).synchronize()
 
     def get_k_pages(self, layer: int):
         """[num_pages, page_size, kv_dim] K pages of a layer."""

@@ -169,6 +169,21 @@ def _slow(stream):
 
 
 @pytest.mark.gpu
+def test_a_new_cache_is_written_before_it_is_used(cuda):
+    """Made behind slow work on torch's stream: its table, lengths and counts stand when the constructor returns."""
+    import torch
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        keep = _slow(side)
+        c = b200attn.PagedKVCache(1, 4, 16, 1, 8, 2, 8)
+        assert side.query()
+    c.extend(c.seq_len[:1].clone(), torch.ones(1, dtype=torch.int32, device="cuda"), stream=None)
+    assert c.check() == 1
+    del keep
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("how", ["stream", "handle", "default", "graph"])
 def test_check_waits_for_the_last_operation(cuda, how):
     """Queued behind slow work on a stream that torch's own does not wait for: its refusal is seen."""
