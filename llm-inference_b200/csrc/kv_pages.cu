@@ -16,7 +16,9 @@
 //
 // extend is one launch as well. The first CTA plans and writes the whole
 // bookkeeping; the others wait for its word (bounded) and copy the shared last
-// pages with it. Its word comes as soon as it is known that none is copied.
+// pages with it. Its word comes as soon as it is known that none is copied. A
+// CTA whose wait runs out (other kernels kept the first CTA from an SM) leaves
+// its share to the CTA that finishes last, which then copies all pages again.
 //
 // The contents move with 16-byte loads and streaming stores, four in flight a
 // thread: HBM-bound, a page's bytes read once and written once. (Plain stores:
@@ -98,7 +100,7 @@ __device__ __forceinline__ uint32_t pieces_of(const Pool& p, uint32_t threads) {
 
 // What the workspace begins with, zero before its first use.
 struct Header {
-    uint32_t finished;  // CTAs of this launch that are done
+    uint32_t finished;  // CTAs of this launch that are done (kGaveUp apiece: and had copied nothing)
     uint32_t word;      // extend: 0, or 1 + the pages to copy
     uint32_t moves;     // pages that this compact moves
     uint32_t unused;
@@ -207,19 +209,23 @@ __device__ __forceinline__ uint32_t hash_slot(Hash& h, int32_t key) {
 }
 static_assert(kHash == 1u << 11, "hash_slot gives 11 bits");
 
-// True in the CTA that comes last; the counter is then 0 again.
-__device__ __forceinline__ bool last_cta(uint32_t* counter, uint32_t* flag) {
+constexpr uint32_t kGaveUp = 1u << 16;  // beside the count of CTAs
+
+// In the CTA that comes last 1 + how many CTAs gave `mark` as kGaveUp, 0 in
+// the others; the counter is then 0 again.
+__device__ __forceinline__ uint32_t last_cta(uint32_t* counter, uint32_t* flag, uint32_t mark = 0u) {
     __syncthreads();
-    if (gridDim.x == 1) return true;
+    if (gridDim.x == 1) return 1u;
     if (threadIdx.x == 0) {
         __threadfence();
-        const uint32_t old = atomicAdd(counter, 1u);
-        *flag = old + 1 == gridDim.x;
-        if (old + 1 == gridDim.x) *counter = 0u;
+        const uint32_t now = atomicAdd(counter, 1u + mark) + 1u + mark;
+        const bool last = (now & (kGaveUp - 1)) == gridDim.x;
+        *flag = last ? 1u + now / kGaveUp : 0u;
+        if (last) *counter = 0u;
         __threadfence();
     }
     __syncthreads();
-    return *flag != 0;
+    return *flag;
 }
 
 // Which of this thread's four pages from page `base` on are free.
@@ -413,6 +419,27 @@ __device__ __forceinline__ void tell(Header* head, uint32_t copies) {
     asm volatile("st.release.gpu.u32 [%0], %1;" ::"l"(&head->word), "r"(copies + 1) : "memory");
 }
 
+__device__ __forceinline__ uint32_t told(const Header* head) {
+    uint32_t word;
+    asm volatile("ld.acquire.gpu.u32 %0, [%1];" : "=r"(word) : "l"(&head->word) : "memory");
+    return word;
+}
+
+// Every `step`th piece of the listed copies, from piece `begin` on.
+__device__ __forceinline__ void copy_listed(const Pool& p, const Header* head, uint32_t copies, uint32_t n,
+                                            uint32_t begin, uint32_t step) {
+    if (copies > n) copies = 0;  // a workspace that was not zero at first: nothing is followed
+    const uint32_t pieces = pieces_of(p, kPlanThreads);
+    for (uint64_t w = begin; w < static_cast<uint64_t>(copies) * pieces; w += step) {
+        const uint32_t c = static_cast<uint32_t>(w / pieces);
+        const uint32_t src = static_cast<uint32_t>(__ldcg(head->lists + c));
+        const uint32_t dst = static_cast<uint32_t>(__ldcg(head->lists + kItems + c));
+        if (src < p.num_pages && dst < p.num_pages)
+            copy_piece(p, src, dst, static_cast<uint32_t>(w - static_cast<uint64_t>(c) * pieces) * kPlanThreads * kCopyUnroll,
+                       kPlanThreads);
+    }
+}
+
 // The whole bookkeeping of an extend, by one CTA. Returns the pages to copy, listed in head.
 __device__ uint32_t extend_plan(ExtendShared& sm, const Seqs& q, const int32_t* seqs, const int32_t* new_tokens,
                                 uint32_t n, int32_t* first, int32_t* status, Header* head) {
@@ -527,7 +554,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(const Pool p, cons
     __shared__ ExtendShared sm;
     pdl_wait_primary();
     pdl_launch_dependents();
-    uint32_t copies;
+    uint32_t copies, gave_up = 0;
     if (blockIdx.x == 0) {
         copies = extend_plan(sm, q, seqs, new_tokens, n, first, status, head);
     } else {
@@ -535,26 +562,25 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(const Pool p, cons
             const uint64_t deadline = global_timer_ns() + kWaitBudgetNs;
             uint32_t word;
             do {
-                asm volatile("ld.acquire.gpu.u32 %0, [%1];" : "=r"(word) : "l"(&head->word) : "memory");
+                word = told(head);
             } while (word == 0 && global_timer_ns() < deadline);
-            if (word == 0) atomicOr(&g_device_error, kErrWaitTimeout);
             sm.s.flag = word;
         }
         __syncthreads();
         copies = sm.s.flag ? sm.s.flag - 1 : 0u;
+        gave_up = sm.s.flag ? 0u : kGaveUp;
     }
-    if (copies > n) copies = 0;  // a workspace that was not zero at first: nothing is followed
-    const uint32_t pieces = pieces_of(p, kPlanThreads);
-    for (uint64_t w = blockIdx.x; w < static_cast<uint64_t>(copies) * pieces; w += gridDim.x) {
-        const uint32_t c = static_cast<uint32_t>(w / pieces);
-        const uint32_t src = static_cast<uint32_t>(__ldcg(head->lists + c));
-        const uint32_t dst = static_cast<uint32_t>(__ldcg(head->lists + kItems + c));
-        if (src < p.num_pages && dst < p.num_pages)
-            copy_piece(p, src, dst, static_cast<uint32_t>(w - static_cast<uint64_t>(c) * pieces) * kPlanThreads * kCopyUnroll,
-                       kPlanThreads);
-    }
+    copy_listed(p, head, copies, n, blockIdx.x, gridDim.x);
     // the last to have read the word takes it back for the next call
-    if (last_cta(&head->finished, &sm.s.flag) && threadIdx.x == 0) head->word = 0u;
+    const uint32_t last = last_cta(&head->finished, &sm.s.flag, gave_up);
+    if (last == 0) return;
+    if (last > 1) {
+        __syncthreads();  // flag is read
+        if (threadIdx.x == 0) sm.s.flag = told(head) - 1;
+        __syncthreads();
+        copy_listed(p, head, sm.s.flag, n, 0, 1);
+    }
+    if (threadIdx.x == 0) head->word = 0u;
 }
 
 // ---- compact ---------------------------------------------------------------------

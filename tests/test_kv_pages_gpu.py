@@ -356,6 +356,32 @@ def test_the_pages_taken_are_counted_when_they_are_too_many(cuda):
     d.same()
 
 
+def test_copies_that_other_ctas_gave_up_are_made(cuda):
+    """The workspace as CTAs leave it whose wait for the plan ran out: they are counted, beside the CTAs
+    that are done, and a word that stands too early has the others copy nothing. The pages are copied
+    all the same, and the workspace is as new."""
+    import torch
+    m = _model(72, 80, 4, 2048, 20, 4)
+    d = Device(m)
+    for s in (m, d):
+        s.extend([0], [10])
+        s.fork([0] * 19, list(range(1, 20)))
+    head = d.ws[0][:16].view(torch.int32)        # finished, word, moves, unused
+    head.copy_(_i32([1 << 16, 1, 0, 0]))
+    _sync()
+    kids = list(range(1, 20))
+    assert d.extend(kids, [1] * 19)[:2] == m.extend(kids, [1] * 19)[:2] == (m.OK, 19)
+    d.same()
+    assert host(head).tolist() == [0] * 4 and _error_word() == 0
+    for s in (m, d):
+        s.truncate(kids, [9] * 19)
+        s.truncate([0])
+        s.fork([1], [0])
+    assert d.extend([0], [1])[:2] == m.extend([0], [1])[:2]
+    d.same()
+    assert host(head).tolist() == [0] * 4
+
+
 def test_on_another_stream_and_captured(cuda):
     """A scheduler's step (drop, fork, extend) captured once, replayed with other items in the same buffers."""
     import torch
