@@ -1,10 +1,14 @@
 """The paged cache without a GPU: the entry points' refusals (all before the
 first CUDA call) and the host model that the GPU tests hold the kernels to."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
 import b200attn
 from _paged import Pages, attend64, rows_of
+from _util import ROOT
 
 F = 0x1000
 
@@ -181,3 +185,45 @@ def test_attend64_known_answer():
     o, b = attend64(q, np.ones((3, 1, 4)), v, 2, 1)
     np.testing.assert_allclose(o, np.tile(v.mean(0), (2, 1)))
     assert np.all(b > 0) and np.all(b < 0.02)
+
+
+SLOT_PAIR = r"""
+#include <cstdio>
+#include "slot_pair.h"
+// A producer of rows, each one copy and then some stages, that gives up before any of its
+// waits: every copy that is issued and not given back is among those that it then waits for.
+int main() {
+    for (int give_up = 0; give_up < 60; ++give_up) {
+        b2::SlotPair q;
+        int phases[2] = {0, 0}, waits = 0, copies = 0;   // phases: copies into each slot
+        bool on = true;
+        for (int row = 0; row < 7 && on; ++row) {
+            if (q.in_use() && waits++ == give_up) break;
+            // the phase that is waited for is the slot's last one
+            if (q.in_use() && q.free_parity() != unsigned(phases[q.next()] - 1) % 2) return 1;
+            q.issue([&](uint32_t s) { ++phases[s]; ++copies; });
+            for (int stage = 0; stage < 3 && on; ++stage) if (waits++ == give_up) on = false;
+        }
+        if (q.issued() != unsigned(copies)) return 2;
+        int pending = 0;
+        for (uint32_t j = q.oldest(); j < q.issued(); ++j, ++pending)
+            if (b2::SlotPair::slot(j) != j % 2 || b2::SlotPair::parity(j) != (j / 2) % 2) return 3;
+        if (pending != (copies < 2 ? copies : 2)) return 4;
+    }
+    return 0;
+}
+"""
+
+
+def test_copies_in_flight_are_counted_as_they_are_issued(tmp_path):
+    """The producer of the tiled decode leaves its loop only with its copies into shared memory done:
+    the count behind that wait is taken by the issue itself, and the producer issues through it."""
+    csrc = os.path.join(ROOT, "llm-inference_b200", "csrc")
+    exe = str(tmp_path / "slots")
+    res = subprocess.run(["g++", "-std=c++17", "-x", "c++", "-", "-o", exe, f"-I{csrc}"], input=SLOT_PAIR,
+                         capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    assert subprocess.run([exe]).returncode == 0
+    with open(os.path.join(csrc, "paged_decode_sm100.cu")) as f:
+        kernel = f.read()
+    assert kernel.count("q_rows.issue(") == 1 and kernel.count("a.q + ") == 1
