@@ -117,14 +117,15 @@ def lib() -> ctypes.CDLL:
 
 
 def calls():
-    """The calls of _native.so (csrc/pycalls.cpp), bound to the loaded library."""
+    """The calls of the _native module (csrc/pycalls.cpp), bound to the loaded library."""
     global _calls
     if _calls is None:
         L = lib()
         try:
             from . import _native
         except ImportError as e:
-            raise RuntimeError("b200attn/_native.so is missing: build it with `python llm-inference_b200/build.py`") from e
+            raise RuntimeError("b200attn/_native, the paged cache's calls, is missing for this interpreter: build it with "
+                               "`python llm-inference_b200/build.py` (g++ and Python's headers)") from e
         for name in _native.NAMES:
             _native.bind(name, ctypes.cast(getattr(L, name), ctypes.c_void_p).value)
         _calls = _native
