@@ -443,6 +443,14 @@ int b2_launch_decode_step_ragged_fused(const void* d_q, size_t q_seq_stride, con
  * or an idle entry is skipped, so is a position past the capacity; with
  * apply_rotation one past rope_rows is skipped and sets bit 1 of the error
  * word. num_heads 0: no query rows. Two rows must not name the same place.
+ * Attending a prompt: b2_launch_causal_attention_prefill reads contiguous rows,
+ * not pages, and after this call the rows hold a rotated Q beside K as it was.
+ * A prompt that starts its sequence is rotated with b2_launch_rope (Q and K),
+ * stored by this call without apply_rotation (num_heads 0), the same bits, and
+ * attended from its rows. Rows that continue a sequence (a chunk, a later turn,
+ * a forked prefix, drafts) are stored by this call and attended by the paged
+ * decode, an entry a row with lengths that grow by one; each entry reads its
+ * whole sequence.
  * 16-byte aligned rows and a head_dim that is a multiple of 16 run the vector
  * kernel, others a scalar one with the same results. */
 int b2_launch_rope_and_store_kv_paged(void* d_q, const void* d_k, const void* d_v, void* d_k_pages,

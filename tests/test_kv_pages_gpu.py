@@ -8,7 +8,7 @@ import b200attn
 import oracle
 from _gpu import Graph, bits, dev, host
 from _paged import Pages, assert_within, attend64, rows_of
-from _util import seeded_f16
+from _util import MAX_ABS, REL_L2, max_abs, rel_l2, seeded_f16
 
 pytestmark = pytest.mark.gpu
 
@@ -531,4 +531,72 @@ def test_a_served_batch(cuda):
     prompts([5, 0], [50, 3])
     step([0, 1, 2, 3, 4, 5])
     check_rows()
+    assert _error_word() == 0
+
+
+@pytest.mark.parametrize("rotate", [True, False])
+def test_prompts_attended_and_continued(cuda, rotate):
+    """The way of a prompt into pages: Q and K rotated in place, stored as they are, attended from the rows;
+    then a chunk that continues one, attended an entry a row. The pages hold what the rotating append stores."""
+    import torch
+    H, KVH, d, ps, pages, rows, stride, cap = 16, 4, 128, 16, 60, 3, 20, 320
+    kv, wide = KVH * d, (H + 2 * KVH) * d
+    cos, sin = b200attn.rope_tables_host(cap, d, 5.0e6)
+    dcos, dsin = dev(cos), dev(sin)
+    c = b200attn.PagedKVCache(1, pages, ps, KVH, d, rows, stride)
+    seqs, lens = [2, 0], [200, 37]
+    x = seeded_f16((sum(lens), wide), 60)
+    qkv = dev(x)
+    out = torch.empty((sum(lens), H * d), dtype=torch.float16, device="cuda")
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    who, at = np.repeat(seqs, lens), np.concatenate([np.arange(n) for n in lens])
+    c.extend(_i32(seqs), _i32(lens), pos)
+    starts = [0, lens[0]]
+    if rotate:
+        for a, n in zip(starts, lens):
+            b200attn.launch_rope(qkv[a:], qkv[a:, H * d:], dcos, dsin, n, H, KVH, d, wide, wide, 0)
+    b200attn.launch_rope_and_store_kv_paged(None, qkv[:, H * d:], qkv[:, H * d + kv:], *c.pages(0), _i32(who), None, None,
+                                            0, sum(lens), 0, KVH, d, 0, wide, _i32(at), False)
+    for a, n in zip(starts, lens):
+        b200attn.launch_causal_attention_prefill(qkv[a:], qkv[a:, H * d:], qkv[a:, H * d + kv:], out[a:], n, H, KVH, d,
+                                                 wide, wide)
+    assert c.check() == 13 + 3 and pos.tolist() == [0, 0]
+    # the same rows through the rotating append
+    other = b200attn.PagedKVCache(1, pages, ps, KVH, d, rows, stride)
+    other.buffer.copy_(c.buffer)
+    other.get_k_pages(0)[:16].zero_()
+    y = dev(x)
+    b200attn.launch_rope_and_store_kv_paged(y, y[:, H * d:], y[:, H * d + kv:], *other.pages(0)[:5], c.page_table, stride,
+                                            rows, _i32(who), dcos, dsin, cap, sum(lens), H, KVH, d, wide, wide, _i32(at),
+                                            rotate)
+    _sync()
+    table = host(c.page_table)
+    kp, vp = (host(p) for p in (c.get_k_pages(0), c.get_v_pages(0)))
+    for s, n in zip(seqs, lens):
+        np.testing.assert_array_equal(bits(rows_of(kp, table[s], n, ps)),
+                                      bits(rows_of(host(other.get_k_pages(0)), table[s], n, ps)))
+    np.testing.assert_array_equal(bits(host(y)[:, :H * d]), bits(host(qkv)[:, :H * d]))
+    q = host(qkv)[:, :H * d].reshape(-1, H, d)
+    for a, s, n in zip(starts, seqs, lens):
+        k, v = (rows_of(p, table[s], n, ps).reshape(n, KVH, d) for p in (kp, vp))
+        want = np.array([attend64(q[a + t], k[:t + 1], v[:t + 1], H, KVH)[0] for t in range(n)]).reshape(n, -1)
+        got = host(out)[a:a + n]
+        assert max_abs(got, want) <= MAX_ABS and rel_l2(got, want) <= REL_L2
+    # nine more rows of sequence 2
+    n, old = 9, 200
+    z = seeded_f16((n, wide), 61)
+    qkv = dev(z)
+    c.extend(_i32([2]), _i32([n]), pos)
+    assert c.check() == 1 and pos.tolist()[0] == old
+    b200attn.launch_rope_and_store_kv_paged(qkv, qkv[:, H * d:], qkv[:, H * d + kv:], *c.pages(0), _i32([2] * n), dcos, dsin,
+                                            cap, n, H, KVH, d, wide, wide, _i32(range(old, old + n)), rotate)
+    size = b200attn.decode_paged_workspace_bytes(n, H, KVH, d)
+    b200attn.launch_causal_attention_decode_paged(qkv, wide, *c.pages(0), _i32([2] * n), _i32(range(old, old + n)), 1, out,
+                                                  0, n, H, KVH, d, torch.zeros(size, dtype=torch.uint8, device="cuda"), size)
+    _sync()
+    table = host(c.page_table)
+    k, v = (rows_of(host(p), table[2], old + n, ps).reshape(-1, KVH, d) for p in (c.get_k_pages(0), c.get_v_pages(0)))
+    for t in range(n):
+        want, bound = attend64(host(qkv)[t, :H * d].reshape(H, d), k[:old + t + 1], v[:old + t + 1], H, KVH)
+        assert_within(host(out)[t].reshape(H, d), want, bound)
     assert _error_word() == 0
