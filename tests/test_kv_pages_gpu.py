@@ -442,6 +442,48 @@ def test_two_streams_at_once(cuda):
     assert _error_word() == 0
 
 
+def test_two_streams_without_waiting(cuda):
+    """Rounds of truncate, fork and extend of two caches, queued on two streams with nothing between
+    them that waits: whole states and every call's positions against the model."""
+    import torch
+    rounds, made = 20, []
+    for k in range(2):
+        m = _model(36, 400, 8, 512, 40, 10, seed=93 + k)
+        d = Device(m)
+        d.stream = torch.cuda.Stream()
+        plan = []
+        for r in range(rounds):
+            seqs = [(3 * r + i + k) % 40 for i in range(30)]
+            take = [1 + (r + i) % 5 for i in range(30)]
+            drop, kids = seqs[15:], seqs[15:]
+            parents = [seqs[i % 15] for i in range(15)]
+            first = torch.full((30,), -77, dtype=torch.int32, device="cuda")
+            plan.append(([_i32(x) for x in (drop, parents, kids, seqs, take)], first, (drop, parents, kids, seqs, take)))
+        made.append((m, d, plan))
+    _sync()
+    for r in range(rounds):
+        for m, d, plan in made:
+            (drop, parents, kids, seqs, take), first, _ = plan[r]
+            s = d.seqs()
+            b200attn.launch_kv_pages_truncate(*s, drop, None, 15, d.status, *d.ws, stream=d.stream)
+            b200attn.launch_kv_pages_fork(*s, parents, kids, None, 15, d.status, *d.ws, stream=d.stream)
+            b200attn.launch_kv_pages_extend(*d.where, *s[:4], *s[5:], seqs, take, 30, first, d.status, *d.ws,
+                                            stream=d.stream)
+    _sync()
+    copies = 0
+    for m, d, plan in made:
+        for _, first, (drop, parents, kids, seqs, take) in plan:
+            assert m.truncate(drop) == m.fork(parents, kids) == m.OK
+            before = m.ref.copy()
+            st, _, want = m.extend(seqs, take)
+            assert st == m.OK
+            copies += int((m.ref < before).sum())     # pages that lost a holder to its copy
+            np.testing.assert_array_equal(host(first), want)
+        d.same()
+        m.check()
+    assert copies > 100 and _error_word() == 0
+
+
 def test_a_served_batch(cuda):
     """Prompts appended, forked into beams, decoded a few steps over two layers through pages,
     rolled back, compacted and decoded on: each output against 64-bit attention of the rows
