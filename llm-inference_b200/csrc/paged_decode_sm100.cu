@@ -254,7 +254,7 @@ __global__ void __maxnreg__(128)
         const Cut cut = Cut::of(total, t.ctas);
         const uint64_t policy = l2_evict_first_policy();
         uint32_t i = 0;               // stages so far
-        SlotPair q_rows;              // lane 0: the segments' Q rows
+        SlotPair q_rows;              // the segments' Q rows
         uint32_t s = 0, round = 0;    // i % stages, i / stages
         uint32_t at = cut.begin(blockIdx.x);
         const uint32_t end = cut.begin(blockIdx.x + 1);
@@ -381,28 +381,28 @@ __global__ void __maxnreg__(128)
                     }
                     if (j == 0) {
                         // behind the first tiles: the segment's Q row and where its result goes
-                        if (lane == 0) {
-                            if (q_rows.in_use()) ok = mbar_wait(&qempty[q_rows.next()], q_rows.free_parity());
-                            if (ok) q_rows.issue([&](uint32_t qs) {
-                                uint8_t* slot = qslots + qs * t.qslot_bytes;
-                                const uint32_t q_bytes = a.num_heads * 256;
-                                uint32_t* meta = reinterpret_cast<uint32_t*>(slot + q_bytes + 256);
-                                meta[0] = b;
-                                meta[1] = whole ? kNoSeg : blockIdx.x + b;   // the partial's number
-                                meta[2] = word;
-                                meta[3] = nt;
-                                const bool rot = kStep && (word & kRowRotate) != 0;
-                                mbar_arrive_expect_tx(&qfull[qs], q_bytes + (rot ? 256u : 0u));
-                                bulk_g2s_plain(slot, a.q + static_cast<uint64_t>(b) * a.q_stride, q_bytes, &qfull[qs]);
-                                if (rot) {
-                                    const uint64_t p = (word & kRowCapped) ? static_cast<uint64_t>(a.kv_len[b]) : len - 1u;
-                                    bulk_g2s_plain(slot + q_bytes, a.cos + p * 64, 128, &qfull[qs]);
-                                    bulk_g2s_plain(slot + q_bytes + 128, a.sin + p * 64, 128, &qfull[qs]);
-                                }
-                            });
+                        if (lane == 0 && q_rows.in_use()) ok = mbar_wait(&qempty[q_rows.next()], q_rows.free_parity());
+                        const uint32_t qs = q_rows.begin();
+                        if (lane == 0 && ok) {
+                            uint8_t* slot = qslots + qs * t.qslot_bytes;
+                            const uint32_t q_bytes = a.num_heads * 256;
+                            uint32_t* meta = reinterpret_cast<uint32_t*>(slot + q_bytes + 256);
+                            meta[0] = b;
+                            meta[1] = whole ? kNoSeg : blockIdx.x + b;   // the partial's number
+                            meta[2] = word;
+                            meta[3] = nt;
+                            const bool rot = kStep && (word & kRowRotate) != 0;
+                            mbar_arrive_expect_tx(&qfull[qs], q_bytes + (rot ? 256u : 0u));
+                            bulk_g2s_plain(slot, a.q + static_cast<uint64_t>(b) * a.q_stride, q_bytes, &qfull[qs]);
+                            if (rot) {
+                                const uint64_t p = (word & kRowCapped) ? static_cast<uint64_t>(a.kv_len[b]) : len - 1u;
+                                bulk_g2s_plain(slot + q_bytes, a.cos + p * 64, 128, &qfull[qs]);
+                                bulk_g2s_plain(slot + q_bytes + 128, a.sin + p * 64, 128, &qfull[qs]);
+                            }
                         }
                         if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) {
                             ok = false;
+                            q_rows.withdraw();
                             break;
                         }
                     }

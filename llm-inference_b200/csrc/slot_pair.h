@@ -1,6 +1,6 @@
 // The count of copies that a producer issues into two slots in turn, copy j
-// into slot j & 1 as that slot's phase j >> 1. issue() counts a copy as it is
-// issued, so that whoever leaves the producer's loop early still finds every
+// into slot j & 1 as that slot's phase j >> 1. A copy gets its slot by being
+// counted, so that whoever leaves the producer's loop early still finds every
 // copy that may be in flight in [oldest(), issued()). Plain C++: the tests
 // compile it for the host.
 #pragma once
@@ -28,11 +28,10 @@ class SlotPair {
     B2_HOST_DEVICE uint32_t free_parity() const { return parity(n - 2); }
     // The oldest copy that may be in flight: those before it gave their slots back.
     B2_HOST_DEVICE uint32_t oldest() const { return n > 2 ? n - 2 : 0; }
-    template <typename F>
-    B2_HOST_DEVICE void issue(F copy) {
-        copy(next());
-        ++n;
-    }
+    // Counts the next copy, which is issued right behind; its slot. withdraw() where it was not issued after
+    // all: a count too high costs a bounded wait, one too low leaves a copy in flight.
+    B2_HOST_DEVICE uint32_t begin() { return slot(n++); }
+    B2_HOST_DEVICE void withdraw() { --n; }
 };
 
 }  // namespace b2
