@@ -53,9 +53,10 @@ constexpr int kPtConsumers = 8;
 constexpr int kPtThreads = (kPtConsumers + 1) * 32;
 constexpr uint32_t kPtMaxSeqs = 1024;   // 32 a lane of the producer warp; 32 * 32 for its search
 constexpr uint32_t kPtMaxCtas = 160;
-// Smaller pages leave most of a 16-token tile empty: 64 sequences of up to 4096 tokens, 16 heads
-// over 4, take 439 / 224 / 153 / 117 us here with pages of 1 / 2 / 3 / 4 tokens, 167 / 150 / 147 /
-// 145 with the split kernel.
+// Smaller pages leave most of a 16-token tile empty. 64 sequences of 1 to 4096 tokens, lengths spread over
+// their logarithm, 4 query heads a KV head and 1 / 2 / 4 / 8 KV heads: pages of 2 tokens 34 / 50 / 81 / 138 us
+// here and 28 / 31 / 55 / 101 with the split kernel, of 3 tokens 25 / 36 / 57 / 95 and 28 / 31 / 54 / 99, of 4
+// tokens 21 / 29 / 44 / 74 and 28 / 31 / 54 / 97.
 constexpr uint32_t kPtMinPage = 4;
 constexpr uint32_t kPtSmemLimit = 226 * 1024;
 constexpr uint32_t kPtMaxStages = 16;
@@ -69,10 +70,12 @@ constexpr uint32_t kRowBits = 0x0fffffffu, kRowRotate = 1u << 28, kRowAppend = 1
 __host__ __device__ constexpr uint32_t pt_npar(uint32_t kvh) { return kPtConsumers / kvh; }  // warps of a KV head
 __host__ __device__ constexpr uint32_t pt_sub(uint32_t kvh) { return kvh < 4 ? 4 / kvh : 1; }  // tiles of a stage
 __host__ __device__ constexpr uint32_t pt_spar(uint32_t kvh) { return pt_npar(kvh) / pt_sub(kvh); }
-// What starting and ending a segment costs, in tiles: about two stages' time
-// (256 sequences of 1 to 4099 tokens, one KV head: 19.3 us; with one stage's
-// 22.5, with three 19.9: the CTA with the most short sequences is last).
-__host__ __device__ constexpr uint32_t pt_begin(uint32_t kvh) { return kvh == 8 ? 1 : 2 * pt_sub(kvh); }
+// What starting and ending a segment costs, in tiles: about two stages' time. 256 slots of 1 to 4099 tokens
+// (lengths spread over their logarithm, a fifth idle) with 0 / 1 / 2 / 3 / 4 stages: 27.6 / 22.7 / 20.0 / 20.1
+// / 21.1 us with one KV head, 32.6 / 30.0 / 26.5 / 25.2 / 26.1 with 2, 47.3 / 44.8 / 43.4 / 43.5 / 43.9 with 4,
+// 81.2 / 80.5 / 80.4 / 81.5 / 81.7 with 8: the CTA with the most short sequences is last. 64 long ones do not
+// notice it from 2 on.
+__host__ __device__ constexpr uint32_t pt_begin(uint32_t kvh) { return 2 * pt_sub(kvh); }
 
 // The cut of `total` units into a range for each CTA: the first `odd` CTAs get
 // per + 1 units, the others per.
@@ -148,9 +151,11 @@ __device__ __forceinline__ void state_join(WarpState& st, const float* at) {
     }
 }
 
-// 128 registers a thread: more make the tiles no faster, and leave the SM fewer
-// for the join's CTAs, which then do not stand ready (one sequence of 64K tokens
-// 27.2 us against 29.1 with 168, one of 300 6.9 against 7.2).
+// 128 registers a thread, 168 without the limit: more leave the SM fewer for the join's CTAs, which then do not
+// stand ready. One sequence of 64K tokens with 1 / 2 / 4 / 8 KV heads: 12.4 / 15.7 / 24.8 / 48.2 us with 128,
+// 13.8 / 17.1 / 27.4 / 48.0 with 168 (144: 12.3 / 15.7 / 27.4 / 48.2). The limit costs 256 slots of one KV head
+// 19.3 us against 19.0 and nothing on 64 long sequences (110.6 and 110.6); with 8 KV heads it spills 10 to 20
+// bytes, without a trace in the times.
 template <uint32_t KVH, bool kStep>
 __global__ void __maxnreg__(128)
     paged_tiled_kernel(const TiledArgs t, const __grid_constant__ CUtensorMap map_k,
