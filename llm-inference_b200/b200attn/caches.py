@@ -67,7 +67,7 @@ class PagedKVCache:
     operations' arguments: contiguous int32 tensors of table rows, lengths and
     counts on the same device (pos and the arrays after the first may be longer). The
     operations are launches (no synchronisation, capturable); ``check`` waits for the
-    last one and reads its status. Calls are ordered on one stream, or by the caller.
+    last truncate, fork, extend or compact and reads its status. Calls are ordered on one stream, or by the caller.
     """
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
@@ -180,8 +180,9 @@ class PagedKVCache:
         launch_kv_pages_copy(*self._pool(), src, dst, self._items(src, dst), stream)
 
     def check(self, stream=None):
-        """Raises if the last truncate, fork or extend was refused; returns status[1]. Waits for the stream that the
-        last operation was launched on, or for ``stream``: the one that a graph of captured operations runs on."""
+        """Raises if the last truncate, fork or extend was refused; returns status[1] (a compact's: the live pages).
+        Waits for the stream that the last of these was launched on, or for ``stream``: the one that a graph of
+        captured operations runs on. A call without items is none."""
         import torch
         device = self.page_table.device
         stream = self._stream if stream is None else stream
