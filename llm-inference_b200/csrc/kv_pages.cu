@@ -26,8 +26,11 @@
 // an SM that loop against 32 that mostly do not: 95.7 against 90; a ring of bulk
 // copies through shared memory: 103.) 90 us is 6.05 TB/s; 24 pages of 72 planes
 // of 16 KB are copied in 11.2 us. Bound by dependent launches: 64 sequences
-// rolled back and extended 8.7 us; 4 prompts dropped, forked into 8 beams and
-// extended 33.8 us, 13.5 of them the copies.
+// rolled back and extended 9.2 us; 4 prompts dropped, forked into 8 beams and
+// extended 33.6 us, 13.5 of them the copies. Bound by one CTA that walks the
+// counts: with 700 / 20,000 / 100,000 / 2,000,000 pages, 95% of them taken from
+// the low end, an extend of 64 sequences 4 / 10 / 29 / 455 us, a compact with
+// nothing to move 8.5 / 23 / 87 / 1,561.
 #include <algorithm>
 
 #include "paged.cuh"

@@ -11,9 +11,11 @@
 // takes one part of one sequence for up to four query heads of a KV head.
 // head_dim / 8 lanes read a token's row as 16-byte pieces and keep q and o in
 // registers in 32 bits; paged_merge_kernel joins the parts. Each K/V byte is read once per four
-// query heads. Bound by its instructions (about 150 for 32 bytes of a lane):
-// 64 sequences of up to 4096 tokens take 142 us with 16 heads over 4 (1.7 TB/s),
-// 249 with 32 over 8 (2.0 TB/s), 52 with 4 over 1 (1.2 TB/s).
+// query heads. Bound by its instructions:
+// 64 sequences of 4096 tokens take 207 us with 16 heads over 4 (2.6 TB/s), 383
+// with 32 over 8 (2.8), 121 with 8 over 2 (2.2), 69 with 4 over 1 (2.0); 520 with
+// 40 over 4 (1.0), whose rows are read three times; 64 of 1 to 4096 tokens,
+// lengths spread over their logarithm, 54 us (1.5 TB/s), 96, 31, 28 and 123.
 #include <math.h>
 
 #include <algorithm>
@@ -29,7 +31,9 @@ constexpr uint32_t kPgHeads = 4;            // query heads of a CTA of the split
 constexpr uint32_t kPgThreads = 128;
 constexpr uint32_t kPgUnroll = 4;           // tokens of a lane group in flight
 constexpr uint32_t kPgMaxSplits = 512;
-constexpr uint32_t kPgPart = 192;           // tokens of a part at least
+// Tokens of a part at least. With 64 / 192 / 512, 16 heads over 4: one sequence of 300 tokens 12.6 / 17 / 23 us,
+// one of 32K 62 / 46 / 59, 64 of 1 to 4096 tokens 58 / 54 / 58.
+constexpr uint32_t kPgPart = 192;
 constexpr uint32_t kPgMergeThreads = 256;
 // The maximum before any score: below every finite one and finite itself, so that a score of -infinity
 // weighs 0, and one that is NaN, which no maximum shows, still makes a NaN of the weight and the output.
@@ -303,9 +307,10 @@ __global__ void __launch_bounds__(kPgMergeThreads) paged_merge_kernel(const Spli
 }
 
 // Most parts of a sequence for the split kernel: 16 CTAs an SM of 148 if all
-// were as long as the longest. (With 8, and parts of any length, 64 sequences of
-// up to 4096 tokens took 160 us instead of 140, a short one alone 49 instead of
-// 18; with 32 parts the joining costs more than the evenness gives.)
+// were as long as the longest. With 8 / 16 / 32, 16 heads over 4: 64 sequences of
+// 1 to 4096 tokens (lengths spread over their logarithm) 73 / 54 / 51 us, 64 of
+// 4096 tokens 213 / 208 / 222; 32 over 8: 126 / 96 / 84 and 383 / 384 / 389; 4
+// over 1: 27.5 / 28 / 30 and 71 / 69 / 71.
 uint32_t paged_splits(size_t num_seqs, size_t num_heads, size_t num_kv_heads) {
     const size_t group = num_heads / num_kv_heads;
     const size_t ctas = num_seqs * num_kv_heads * ((group + kPgHeads - 1) / kPgHeads);

@@ -25,9 +25,9 @@
 // * paged_join_kernel joins the partials of the sequences that were cut.
 //
 // Measured, a call in a graph: 64 sequences of 512 to 16K tokens, 16 heads over
-// 4, 111 us (6.45 TB/s, the copy peak 6.55); one of 64K 27.3 us (4.9 TB/s: 3.5
-// until the first tile, 5 for flush and join); 256 of one KV head 19.5; a step
-// of 48 with 8 KV heads 78.6 (6.07 TB/s); one of 300 tokens 6.8.
+// 4, 111.4 us (6.45 TB/s, the copy peak 6.55); one of 64K 27.7 us (4.8 TB/s: 3.5
+// until the first tile, 5 for flush and join); 256 of one KV head 19.6; a step
+// of 48 with 8 KV heads 78.2 (6.1 TB/s); one of 300 tokens 7.0.
 //
 // The weights go to the tensor cores as two 16-bit numbers each (kWide of
 // tile_softmax_pv: off by 2^-22 of a weight, or by 2^-32 of the largest);
