@@ -474,7 +474,7 @@ int b2_launch_rope_and_store_kv_paged(void* d_q, const void* d_k, const void* d_
  * query heads each, num_seqs <= 1024, pages of 4 tokens or more, an even
  * out_seq_stride and num_seqs * table_stride * ceil(page_size / 16) below
  * about 2^31 run the tensor-core kernel; other calls run a SIMT kernel at a
- * fifth to a third of its rate. d_workspace: b2_decode_paged_workspace_bytes bytes
+ * sixth (many query heads a KV head) to two fifths of its rate. d_workspace: b2_decode_paged_workspace_bytes bytes
  * (whatever the lengths; it needs no initial contents); one workspace serves
  * calls ordered on one stream. The result depends on the call's inputs alone,
  * bit for bit. */
