@@ -62,6 +62,7 @@ size_t b2_decode_workspace_floats(size_t num_heads, size_t head_dim, size_t max_
 const char* b2_status_string(int status);
 int b2_last_cuda_error(void);            /* cudaError_t of the last B2_ERR_CUDA */
 uint64_t b2_kernel_launch_count(void);   /* kernels this library has launched */
+int b2_current_device(void);             /* the device that launches go to; -1 without one */
 /* OR of the device-side error bits on the current device: bit 0 = a bounded
  * wait inside a kernel (TMA copy / pipeline barrier) ran out of time and the
  * kernel stopped early; bit 1 = a fused decode step got a RoPE position

@@ -31,6 +31,7 @@ SIGNATURES: dict[str, tuple] = {
     "b2_status_string": (ctypes.c_char_p, [I]),
     "b2_last_cuda_error": (I, []),
     "b2_kernel_launch_count": (U64, []),
+    "b2_current_device": (I, []),
     "b2_device_error_word": (ctypes.c_uint, []),
     "b2_clear_device_error_word": (I, []),
     "b2_fill_rope_tables": (I, [S, S, F, P, P]),
@@ -126,7 +127,7 @@ def calls():
         except ImportError as e:
             raise RuntimeError("b200attn/_native, the paged cache's calls, is missing for this interpreter: build it with "
                                "`python llm-inference_b200/build.py` (g++ and Python's headers)") from e
-        for name in _native.NAMES:
+        for name in [*_native.NAMES, "b2_current_device"]:
             _native.bind(name, ctypes.cast(getattr(L, name), ctypes.c_void_p).value)
         _calls = _native
     return _calls

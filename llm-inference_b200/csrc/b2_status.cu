@@ -71,6 +71,13 @@ int b2_last_cuda_error(void) { return b2::g_last_cuda_error.load(); }
 
 uint64_t b2_kernel_launch_count(void) { return b2::g_launches.load(); }
 
+int b2_current_device(void) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) == cudaSuccess) return dev;
+    (void)cudaGetLastError();
+    return -1;
+}
+
 unsigned int b2_device_error_word(void) {
     return b2::device_error_decode() | b2::device_error_prefill() | b2::device_error_ragged() |
            b2::device_error_proj() | b2::device_error_append() | b2::device_error_paged() | b2::device_error_pages();

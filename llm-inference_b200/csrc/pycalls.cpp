@@ -2,8 +2,10 @@
 // ctypes: a call of 24 arguments spends 13 us in ctypes and in taking the
 // tensors' addresses in Python, more than the smallest kernels run; here it
 // takes about 2. The arguments are converted by the C declarations' types:
-// device pointers from a tensor (its data_ptr(), host tensors are refused), an
-// int or None; streams from a torch stream (its cuda_stream), an int or None.
+// device pointers from a tensor (its data_ptr(); host tensors are refused, so
+// are those of another device than the current one, which the kernels could not
+// read), an int or None; streams from a torch stream (its cuda_stream), an int
+// or None.
 //
 // The module does not link the library: bind(name, address) gives it the
 // functions of the one that _lib.py has loaded.
@@ -20,8 +22,45 @@
 namespace {
 
 PyObject* s_is_cuda;
+PyObject* s_get_device;
 PyObject* s_data_ptr;
 PyObject* s_cuda_stream;
+
+int (*fn_current_device)(void) = nullptr;
+constexpr int kNotAsked = -2;
+thread_local int current_device = kNotAsked;  // in this call
+
+// A host tensor is refused, so is one of another device. Objects that know neither pass.
+bool on_current_device(PyObject* o) {
+    PyObject* d = PyObject_CallMethodNoArgs(o, s_get_device);
+    long device = -1;
+    if (d != nullptr) {
+        device = PyLong_AsLong(d);
+        Py_DECREF(d);
+        if (device == -1 && PyErr_Occurred()) return false;
+    } else if (PyErr_ExceptionMatches(PyExc_AttributeError)) {
+        PyErr_Clear();
+        PyObject* cuda = PyObject_GetAttr(o, s_is_cuda);
+        if (cuda == nullptr) {
+            if (!PyErr_ExceptionMatches(PyExc_AttributeError)) return false;
+            PyErr_Clear();
+            return true;
+        }
+        const bool host = cuda == Py_False;
+        Py_DECREF(cuda);
+        if (!host) return true;
+    } else {
+        return false;
+    }
+    if (device < 0) {
+        PyErr_SetString(PyExc_ValueError, "b200attn launchers take device buffers; got a host tensor");
+        return false;
+    }
+    if (current_device == kNotAsked) current_device = fn_current_device ? fn_current_device() : -1;
+    if (device == current_device) return true;
+    PyErr_Format(PyExc_ValueError, "a tensor lies on device %ld, the current device is %d", device, current_device);
+    return false;
+}
 
 bool convert(PyObject* o, void*& out) {
     if (o == Py_None) {
@@ -32,18 +71,7 @@ bool convert(PyObject* o, void*& out) {
         out = PyLong_AsVoidPtr(o);
         return out != nullptr || !PyErr_Occurred();
     }
-    PyObject* cuda = PyObject_GetAttr(o, s_is_cuda);
-    if (cuda == nullptr) {
-        if (!PyErr_ExceptionMatches(PyExc_AttributeError)) return false;
-        PyErr_Clear();
-    } else {
-        const bool host = cuda == Py_False;
-        Py_DECREF(cuda);
-        if (host) {
-            PyErr_SetString(PyExc_ValueError, "b200attn launchers take device buffers; got a host tensor");
-            return false;
-        }
-    }
+    if (!on_current_device(o)) return false;
     PyObject* p = PyObject_CallMethodNoArgs(o, s_data_ptr);
     if (p == nullptr) {
         if (PyErr_ExceptionMatches(PyExc_AttributeError)) {
@@ -110,6 +138,7 @@ PyObject* call(int (*fn)(A...), const char* name, PyObject* const* args, Py_ssiz
                      static_cast<int>(n));
         return nullptr;
     }
+    current_device = kNotAsked;
     std::tuple<A...> v{};
     if (!(convert(args[I], std::get<I>(v)) && ...)) return nullptr;
     int status;
@@ -150,6 +179,10 @@ PyObject* bind(PyObject*, PyObject* args) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null function");
         return nullptr;
     }
+    if (std::string_view(name) == "b2_current_device") {
+        fn_current_device = reinterpret_cast<int (*)(void)>(p);
+        Py_RETURN_NONE;
+    }
 #define B2_BIND(f)                                          \
     if (std::string_view(name) == #f) {                     \
         fn_##f = reinterpret_cast<decltype(fn_##f)>(p);     \
@@ -171,9 +204,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "calls of libb200attn.so
 
 PyMODINIT_FUNC PyInit__native(void) {
     s_is_cuda = PyUnicode_InternFromString("is_cuda");
+    s_get_device = PyUnicode_InternFromString("get_device");
     s_data_ptr = PyUnicode_InternFromString("data_ptr");
     s_cuda_stream = PyUnicode_InternFromString("cuda_stream");
-    if (!s_is_cuda || !s_data_ptr || !s_cuda_stream) return nullptr;
+    if (!s_is_cuda || !s_get_device || !s_data_ptr || !s_cuda_stream) return nullptr;
     PyObject* m = PyModule_Create(&module);
     if (m == nullptr) return nullptr;
     PyObject* names = Py_BuildValue("[" 

@@ -93,6 +93,39 @@ def test_native_calls_refuse_what_they_cannot_pass():
     f(0x1000, 1, 0, 1, 0, 8, 0x1000, 0x1000, 0)           # nothing to do
 
 
+class _Elsewhere:
+    """A tensor of a device that is not the current one, as far as a call looks at it."""
+    is_cuda = True
+
+    def get_device(self):
+        return 63
+
+    def data_ptr(self):
+        return 0x1000
+
+
+def test_native_calls_refuse_tensors_of_another_device():
+    """With no items, so that nothing runs either way."""
+    a, x = 0x1000, _Elsewhere()
+    for call in (lambda: b200attn.launch_kv_pages_copy(a, 1, 0, 1, 0, 8, a, x, 0),
+                 lambda: b200attn.launch_kv_pages_truncate(x, 1, 1, 1, 1, a, a, a, a, 0, a, a, 0),
+                 lambda: b200attn.launch_rope_and_store_kv_paged(x, a, a, a, a, 0, 1, 1, a, 1, 1, a, a, a, 1, 0, 1, 1, 8, 0,
+                                                                 0, a, True),
+                 lambda: b200attn.launch_causal_attention_decode_paged(a, 0, a, x, 0, 1, 1, a, 1, 1, a, a, 0, a, 0, 0, 1, 1,
+                                                                       8, a, 0)):
+        with pytest.raises(ValueError, match="device 63"):
+            call()
+
+
+@pytest.mark.gpu
+def test_native_calls_on_the_current_device(cuda):
+    import torch
+    t = torch.zeros(8, dtype=torch.int32, device="cuda")
+    assert b200attn.lib().b2_current_device() == torch.cuda.current_device() == t.get_device()
+    b200attn.launch_kv_pages_copy(t, 1, 0, 1, 0, 8, t, t, 0)
+    test_native_calls_refuse_tensors_of_another_device()
+
+
 def test_cpp_class_compiles():
     src = ('#include "b200attn/paged_kv_cache.hpp"\n'
            'int main() { return sizeof(b200attn::PagedKVCache) == 0 || &b200attn::PagedKVCache::compact == nullptr; }\n')
