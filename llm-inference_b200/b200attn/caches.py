@@ -92,9 +92,11 @@ class PagedKVCache:
         if self._ws_bytes == 0:
             raise ValueError(f"{num_pages} pages: 1 to 2**21 are possible")
         self._ws = torch.zeros(self._ws_bytes, dtype=torch.uint8, device=device)
-        self._stream = None   # the last operation's
+        self._device = self._ws.device
+        self._stream = None      # the last operation's
+        self._streams = set()    # those other than torch's own that have used the cache
         if self._ws.is_cuda:   # written before a stream that does not wait for torch's uses them
-            torch.cuda.current_stream(self._ws.device).synchronize()
+            torch.cuda.current_stream(self._device).synchronize()
 
     def get_k_pages(self, layer: int):
         """[num_pages, page_size, kv_dim] K pages of a layer."""
@@ -114,11 +116,11 @@ class PagedKVCache:
     def _table(self):
         return self.page_table, self.max_pages_per_seq, self.max_seqs, self.page_size
 
-    def _items(self, *arrays):
+    def _items(self, stream, *arrays):
         """Items of a call: elements of its first array. The others hold as many
         at least, or the kernels would read past their ends."""
         import torch
-        n, device = arrays[0].numel(), self.page_table.device
+        n, device = arrays[0].numel(), self._device
         for t in arrays:
             if t is None:
                 continue
@@ -126,11 +128,39 @@ class PagedKVCache:
                 raise ValueError(f"expected {n} contiguous int32 on {device}; got {t.numel()} "
                                  f"{'' if t.is_contiguous() else 'strided '}{t.dtype} on {t.device}")
         self._current()
+        self._used_on(stream, *arrays)
         return n
+
+    def _used_on(self, stream, *arrays):
+        """The memory of arrays, and of the cache, that die before a stream other than torch's own is done with them
+        is not given out again (what a graph holds lives as long as the graph: its maker sees to that)."""
+        import torch
+        handle = self._handle(stream)
+        # (the raw handle: torch.cuda.current_stream takes as long as all the rest of a call)
+        if not self._ws.is_cuda or handle == torch._C._cuda_getCurrentRawStream(self._device.index):
+            return
+        with torch.cuda.stream(self._torch_stream(stream)):
+            if torch.cuda.is_current_stream_capturing():
+                return
+            if handle not in self._streams:
+                self._streams.add(handle)
+                arrays += (self.buffer, self.page_table, self.seq_len, self.ref_count, self.status, self._ws)
+            for t in arrays:
+                if t is not None:
+                    t.record_stream(torch.cuda.current_stream(self._device))
+
+    @staticmethod
+    def _handle(stream):
+        return (stream if isinstance(stream, int) else stream.cuda_stream) if stream is not None else 0
+
+    def _torch_stream(self, stream):
+        import torch
+        device, handle = self._device, self._handle(stream)
+        return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
 
     def _current(self):
         import torch
-        device = self.page_table.device
+        device = self._device
         if device.type == "cuda" and device.index != torch.cuda.current_device():
             raise ValueError(f"the cache lies on {device}, which is not the current device")
 
@@ -145,7 +175,7 @@ class PagedKVCache:
     def extend(self, seqs, new_tokens, pos=None, stream=None):
         """Room for new_tokens[i] more tokens of sequence seqs[i]; pos[i] = its first new position."""
         from .kernels import launch_kv_pages_extend
-        n = self._items(seqs, new_tokens, pos)
+        n = self._items(stream, seqs, new_tokens, pos)
         launch_kv_pages_extend(*self._pool(), *self._table(), self.seq_len, self.ref_count, seqs, new_tokens,
                                n, pos, *self._work(stream))
         self._launched(n, stream)
@@ -153,7 +183,7 @@ class PagedKVCache:
     def truncate(self, seqs, new_len=None, stream=None):
         """Sequence seqs[i] keeps its first new_len[i] tokens (None: it is freed)."""
         from .kernels import launch_kv_pages_truncate
-        n = self._items(seqs, new_len)
+        n = self._items(stream, seqs, new_len)
         launch_kv_pages_truncate(*self._table(), self.num_pages, self.seq_len, self.ref_count, seqs, new_len,
                                  n, *self._work(stream))
         self._launched(n, stream)
@@ -161,7 +191,7 @@ class PagedKVCache:
     def fork(self, parents, children, fork_len=None, stream=None):
         """Empty sequence children[i] shares the first fork_len[i] tokens (None: all) of parents[i]."""
         from .kernels import launch_kv_pages_fork
-        n = self._items(parents, children, fork_len)
+        n = self._items(stream, parents, children, fork_len)
         launch_kv_pages_fork(*self._table(), self.num_pages, self.seq_len, self.ref_count, parents, children,
                              fork_len, n, *self._work(stream))
         self._launched(n, stream)
@@ -170,6 +200,7 @@ class PagedKVCache:
         """Brings the live pages together at the low numbers; status[1] = how many they are."""
         from .kernels import launch_kv_pages_compact
         self._current()
+        self._used_on(stream)
         launch_kv_pages_compact(*self._pool(), self.page_table, *self._table(), self.seq_len, self.ref_count,
                                 self.ref_count, *self._work(stream))
         self._launched(1, stream)
@@ -177,19 +208,15 @@ class PagedKVCache:
     def copy_pages(self, src, dst, stream=None):
         """Contents of page dst[i] = those of page src[i], every layer."""
         from .kernels import launch_kv_pages_copy
-        launch_kv_pages_copy(*self._pool(), src, dst, self._items(src, dst), stream)
+        launch_kv_pages_copy(*self._pool(), src, dst, self._items(stream, src, dst), stream)
 
     def check(self, stream=None):
         """Raises if the last truncate, fork or extend was refused; returns status[1] (a compact's: the live pages).
         Waits for the stream that the last of these was launched on, or for ``stream``: the one that a graph of
         captured operations runs on. A call without items is none."""
-        import torch
-        device = self.page_table.device
         stream = self._stream if stream is None else stream
-        if device.type == "cuda":
-            handle = stream if stream is None or isinstance(stream, int) else stream.cuda_stream
-            (torch.cuda.ExternalStream(handle, device=device) if handle
-             else torch.cuda.default_stream(device)).synchronize()
+        if self.page_table.is_cuda:
+            self._torch_stream(stream).synchronize()
         code, count = self.status.tolist()
         if code == 1:
             raise MemoryError(f"too few free pages: the call takes {count}")

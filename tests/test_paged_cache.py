@@ -191,14 +191,60 @@ def test_cpp_class_on_a_non_blocking_stream(cuda, tmp_path):
     assert res.returncode == 0, res.stdout + res.stderr
 
 
-def _slow(stream):
-    """Ordinary work of some 30 ms on a stream."""
+def _slow(stream, rounds=40):
+    """Ordinary work on a stream: some 0.7 ms a round."""
     import torch
     with torch.cuda.stream(stream):
         a = torch.randn(8192, 8192, device="cuda", dtype=torch.bfloat16)
-        for _ in range(40):
+        for _ in range(rounds):
             a = (a @ a).clamp(-1, 1)
     return a
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("default", [False, True])
+def test_arrays_outlive_a_call_on_another_stream(cuda, default):
+    """Arguments dropped while their operation still waits behind slow work on its stream: their
+    memory is not given to the next tensors before."""
+    import torch
+
+    def ints(x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+    warm = b200attn.PagedKVCache(1, 40, 16, 1, 8, 4, 8)     # loading a kernel may wait for the device
+    for call in (warm.extend, warm.fork, warm.truncate, warm.copy_pages):
+        call(ints([-1]), ints([-1]))
+    b200attn.lib().b2_clear_device_error_word()
+    c = b200attn.PagedKVCache(1, 40, 16, 1, 8, 4, 8)
+    pos = ints([-5, -5])
+    side = torch.cuda.default_stream() if default else torch.cuda.Stream()
+    stream = None if default else side
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        # (nothing here waits for the side stream: values come by device copies and fills)
+        zero, two, three, n0, n1 = (torch.full((1,), v, dtype=torch.int32, device="cuda") for v in (0, 2, 3, 20, 33))
+        torch.cat([zero, two])                       # (its kernel is loaded)
+        torch.cuda.current_stream().synchronize()
+        keep = _slow(side, 300)
+        c.extend(torch.cat([zero, two]), torch.cat([n0, n1]), pos, stream=stream)
+        c.fork(torch.cat([two]), torch.cat([three]), torch.cat([n0]), stream=stream)
+        c.truncate(torch.cat([zero]), torch.cat([three]), stream=stream)
+        c.copy_pages(torch.cat([two]), torch.cat([n1]), stream=stream)
+        gone = b200attn.PagedKVCache(1, 40, 16, 1, 8, 4, 8)
+        gone.extend(zero, n0, stream=stream)
+        at = {t.data_ptr() for t in (gone.buffer, gone.page_table, gone.seq_len, gone.ref_count, gone.status, gone._ws)}
+        del gone
+        others = [torch.full((k,), 1, dtype=torch.int32, device="cuda") for _ in range(16) for k in (1, 2)]
+        again = b200attn.PagedKVCache(1, 40, 16, 1, 8, 4, 8)
+        assert not at & {t.data_ptr() for t in (again.buffer, again.page_table, again.seq_len, again.ref_count, again.status,
+                                                again._ws, *others)}
+        torch.cuda.current_stream().synchronize()
+        assert not side.query()                      # all of it was still to come
+        assert c.check() == 0
+    torch.cuda.synchronize()
+    assert c.seq_len.tolist() == [3, 0, 33, 20] and pos.tolist() == [0, 0]
+    assert torch.equal(c.buffer[:, 33].view(torch.int16), c.buffer[:, 2].view(torch.int16))
+    del keep, others
 
 
 @pytest.mark.gpu
